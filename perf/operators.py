@@ -27,8 +27,9 @@ _LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
 def _nsa():
-    if "nsa" not in sys.modules:
-        sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "nsa-test_amd"))
+    p = str(Path(__file__).resolve().parents[1] / "nsa-test_amd")
+    if p not in sys.path:
+        sys.path.insert(0, p)
     import nsa
 
     return nsa
