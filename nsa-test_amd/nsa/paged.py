@@ -447,7 +447,7 @@ class NSAPagedKVCache:
 
     @property
     def K_cmp(self) -> torch.Tensor:
-        """Compressed keys [B,G,dk,blocks] in the layer's dtype (zeros or older ones past a sequence's own)."""
+        """Compressed keys [B,G,dk,blocks] in the layer's dtype (zeros past a sequence's own)."""
         return self._K_cmp[:, :, :-1].transpose(-1, -2)
 
     def check(self, new: Sequence[int], x: Optional[torch.Tensor] = None, config=None) -> None:
@@ -608,3 +608,5 @@ class NSAPagedKVCache:
         _need(0 <= b < self.batch, f"sequence {b} of {self.batch}")
         self._tokens.release(b)
         self._blocks.release(b)
+        # a request without a completed block is scored against block 0, which must not be the last one's
+        self._K_cmp[b].zero_()

@@ -240,3 +240,11 @@ def test_restated_format():
     tab, slots, pos, seq, off, lens, info = ref.tables([[7, -1], [-1, -1]], [15, 0], [3, 1], [4, 5, 6], 1, 16, 4, 0)
     assert tab == [[7, 5], [6, -1]] and slots == [7 * 16 + 15, 5 * 16, 5 * 16 + 1, 6 * 16]
     assert pos == [15, 16, 17, 0] and seq == [0, 0, 0, 1] and off == [0, 3, 4] and lens == [18, 1] and info == [4, 3, 0]
+
+
+def test_release_clears_the_compressed_keys():
+    cfg = nsa.NSAConfig(d_model=64, head_dim_qk=32, head_dim_v=32, n_heads=4, n_kv_groups=2)
+    c = nsa.NSAPagedKVCache(cfg, 2, 100, "cpu", torch.float32, 16)
+    c._K_cmp.fill_(float("nan"))
+    c.release(1)
+    assert not c.K_cmp[1].any() and c.K_cmp[0].isnan().all()
