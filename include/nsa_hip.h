@@ -610,7 +610,8 @@ int nsa_kv4_load(const nsa_kv4_pages* pages, const int32_t* tables, int64_t stri
  *      without any block takes block p / block_size_selection
  *   2  the last window_size positions up to p
  * each read through its own pool and table (tables[s] [Z] rows of table_width[s] entries; a key
- * whose page the table does not name is not there); a source without a pool (null) is absent.  With
+ * whose page the table does not name is not there; one table for sources 1 and 2 means pools of one
+ * page size); a source without a pool (null) is absent.  With
  * gates [Z,H,n_ctx_q,3] (dtype, strides z, h, row, gate; gate_act as in nsa_gate_mix_fwd) out = sum_s
  * act(gate_s) o_s over the present sources, o_s zero where a row sees no key; without (null),
  * exactly one source is present and out = o_s.  Sums and mix in fp32, out rounded to dtype once.

@@ -721,6 +721,8 @@ static int kv4_attn_shape(const nsa_kv4_attn_args& x, Kv4Attn& a) {
     a.parts[s] = 1;
   }
   if (!present) return set_error(NSA_ERR_INVALID, "no source");
+  if (x.pages[1] && x.pages[2] && x.tables[1] && x.tables[1] == x.tables[2] && a.src[1].pg.shift != a.src[2].pg.shift)
+    return set_error(NSA_ERR_INVALID, "one block table for pools of different page sizes");
   if (x.pages[0] && (x.l < 1 || x.d < 1)) return set_error(NSA_ERR_INVALID, "bad l or d");
   if (x.pages[1] && (x.n_slots < 1 || x.n_slots > 64 || x.block_size_selection < 16 ||
                        x.block_size_selection % 16 || x.block_size_selection > (1 << 20)))

@@ -322,11 +322,13 @@ def nsa_attend_kv4(q: torch.Tensor, cmp: PagedKV4, sel: PagedKV4, win: PagedKV4,
                    config, max_length: Optional[int] = None) -> torch.Tensor:
     """The attention of an NSA layer over 4-bit pages: the compressed tokens completed at each query's
     position (cmp through cmp_tables), its selected blocks (sel) and its window (win; sel and win
-    share tables), each as attend_kv4 takes them, mixed by the activated gates [B,H,T,3] (config's
+    share tables and have pages of one size), each as attend_kv4 takes them, mixed by the activated gates [B,H,T,3] (config's
     gate_mode), in one pass.  A branch that sees nothing adds zero."""
     c = config
     if c.l_prime % 16:
         raise ValueError(f"l_prime {c.l_prime} must be a multiple of 16")
+    if sel.page_size != win.page_size:  # the table's pages would stand for other tokens in one of them
+        raise ValueError(f"sel and win share tables, but have pages of {sel.page_size} and {win.page_size} tokens")
     return _attend(q, ((cmp, cmp_tables), (sel, tables), (win, tables)), lengths, scale, c.w, indices, c.l_prime, c.l, c.d, gates,
                    GATE_ACT[c.gate_mode], max_length)
 

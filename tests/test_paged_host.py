@@ -248,3 +248,20 @@ def test_release_clears_the_compressed_keys():
     c._K_cmp.fill_(float("nan"))
     c.release(1)
     assert not c.K_cmp[1].any() and c.K_cmp[0].isnan().all()
+
+
+def test_pools_of_one_table_have_pages_of_one_size():
+    cfg = nsa.NSAConfig(d_model=64, head_dim_qk=64, head_dim_v=64, n_heads=4, n_kv_groups=2, n=4)
+    cmp, sel, win = (nsa.PagedKV4.empty(3, p, 2, 64, 64, "cpu") for p in (64, 16, 32))
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q, idx, z = torch.zeros(1, 4, 1, 64), torch.zeros(1, 2, 1, 4, dtype=torch.int64), torch.zeros(1, 4, 1, 3)
+    with pytest.raises(ValueError, match="pages of 16 and 32"):
+        nsa.nsa_attend_kv4(q, cmp, sel, win, t, t, n, idx, z, 1.0, cfg)
+    with pytest.raises(RuntimeError, match="GPU"):  # (the compressed tokens' table is another)
+        nsa.nsa_attend_kv4(q, cmp, sel, sel, t, t, n, idx, z, 1.0, cfg)
+    lib, a, other = _lib.load(), _attn(sel=False, gates=4096, gate_act=1, indices=4096), _pages(page_size=32)
+    assert lib.nsa_kv4_attn_workspace_size(ctypes.byref(a)) > 0
+    a.pages[1] = ctypes.addressof(other)
+    assert lib.nsa_kv4_attn(ctypes.byref(a), ONE, 1 << 30, None) == 1 and "page sizes" in _err()
+    a.tables[1] = 8192  # a table of its own
+    assert lib.nsa_kv4_attn_workspace_size(ctypes.byref(a)) > 0
