@@ -13,7 +13,8 @@ between steps when every request has its own length.
   with their gates.
 
 The functions take lengths, counts and tables from the device and wait for nothing, so that a step
-of them can be captured into a graph and replayed.  None of it is differentiable.
+of them can be captured into a graph and replayed.  None of it is differentiable: tensors that
+require a gradient are refused outside torch.no_grad().
 """
 from __future__ import annotations
 
@@ -58,6 +59,11 @@ def _refuse(name: str, t: torch.Tensor, want: str) -> None:
     if not t.is_cuda:
         raise RuntimeError("NSA kernels run on the GPU only: got a tensor on " + str(t.device))
     raise ValueError(f"{name} must be {want}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _refuse_grad(name: str) -> None:
+    # the calls work on addresses: a gradient that is asked for would be lost
+    raise RuntimeError(f"{name} is not differentiable: call it under torch.no_grad(), or detach its tensors")
 
 
 def _check_vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, dev: int) -> None:
@@ -188,6 +194,8 @@ def store_kv4(kv: PagedKV4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tenso
     infinity or NaN becomes NaN.  Slots below 0 or outside the pool are skipped; of rows that name
     one slot twice, one of them is there, block by block."""
     N, dev = slots.shape[0] if slots.dim() else 0, kv._dev
+    if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+        _refuse_grad("store_kv4")
     if dev < 0:
         _refuse("the pool", kv.k, "on the GPU")
     _check_vector("slots", slots, N, torch.int64, dev)
@@ -236,6 +244,8 @@ def _attend(q, sources, lengths, scale, window=1, indices=None, block_size=64, l
     """The call of nsa_kv4_attn: sources (pool, tables) or (None, None), three of them in the order of the gates."""
     kv = sources[2][0] or sources[1][0]
     dev, G, (DK, DV), (dk, dv) = kv._kind
+    if (q.requires_grad or gates is not None and gates.requires_grad) and torch.is_grad_enabled():
+        _refuse_grad("attention over 4-bit pages")
     if dev < 0:
         _refuse("the pool", kv.k, "on the GPU")
     if q.dim() != 4 or q.get_device() != dev:

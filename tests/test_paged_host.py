@@ -265,3 +265,19 @@ def test_pools_of_one_table_have_pages_of_one_size():
     assert lib.nsa_kv4_attn(ctypes.byref(a), ONE, 1 << 30, None) == 1 and "page sizes" in _err()
     a.tables[1] = 8192  # a table of its own
     assert lib.nsa_kv4_attn_workspace_size(ctypes.byref(a)) > 0
+
+
+def test_gradients_are_refused():
+    cfg = nsa.NSAConfig(d_model=64, head_dim_qk=64, head_dim_v=64, n_heads=4, n_kv_groups=2, n=4)
+    kv = nsa.PagedKV4.empty(3, 16, 2, 64, 64, "cpu")
+    t, n = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    q, idx, z = torch.zeros(1, 4, 1, 64), torch.zeros(1, 2, 1, 4, dtype=torch.int64), torch.zeros(1, 4, 1, 3)
+    rows, slots = torch.zeros(1, 2, 64), torch.zeros(1, dtype=torch.int64)
+    calls = {"q": lambda x: nsa.attend_kv4(x(q), kv, t, n, 1.0), "nsa q": lambda x: nsa.nsa_attend_kv4(x(q), kv, kv, kv, t, t, n, idx, z, 1.0, cfg),
+             "gates": lambda x: nsa.nsa_attend_kv4(q, kv, kv, kv, t, t, n, idx, x(z), 1.0, cfg),
+             "k": lambda x: nsa.store_kv4(kv, x(rows), rows, slots), "v": lambda x: nsa.store_kv4(kv, rows, x(rows), slots)}
+    for name, f in calls.items():
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            f(lambda y: y.clone().requires_grad_())
+        with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # (on to the next check)
+            f(lambda y: y.clone().requires_grad_())
