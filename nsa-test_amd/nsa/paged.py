@@ -29,6 +29,9 @@ from . import _lib, _ops
 PAGE_SIZES = (16, 32, 64, 128, 256, 512, 1024)
 MAX_REQUESTS = 4096
 MAX_BLOCKS = 4096  # compressed blocks a query can score
+MAX_PAIRS = 65535  # (request, group) pairs of a call
+MAX_BLOCK_SIZE = 1 << 20  # tokens of a selection block
+MAX_TOKENS = 1 << 30  # tokens of a block table
 
 
 # A call of these is one or two launches of a few us each, so its host side is what a step waits
@@ -425,6 +428,10 @@ class NSAPagedKVCache:
         _need(page_size in PAGE_SIZES, f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         _need(1 <= c.n <= 64 and c.heads_per_group <= 64, f"n {c.n} or {c.heads_per_group} heads a group outside [1, 64]")
         _need(batch <= MAX_REQUESTS, f"batch {batch} exceeds {MAX_REQUESTS}")
+        # what the kernels of a decode step would refuse once its token is stored
+        _need(batch * c.n_kv_groups <= MAX_PAIRS, f"{batch} sequences of {c.n_kv_groups} groups: more than {MAX_PAIRS} pairs")
+        _need(c.l_prime <= MAX_BLOCK_SIZE, f"l_prime {c.l_prime} exceeds {MAX_BLOCK_SIZE}")
+        _need(-(-max_len // page_size) * page_size <= MAX_TOKENS, f"max_len {max_len} exceeds {MAX_TOKENS} tokens")
         _need(_n_blocks(max_len, c.l, c.d) <= MAX_BLOCKS,
               f"{max_len} tokens make {_n_blocks(max_len, c.l, c.d)} compressed blocks, the scoring takes {MAX_BLOCKS}")
         self.batch, self.max_len, self.page_size = batch, max_len, page_size

@@ -281,3 +281,19 @@ def test_gradients_are_refused():
             f(lambda y: y.clone().requires_grad_())
         with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # (on to the next check)
             f(lambda y: y.clone().requires_grad_())
+
+
+def test_cache_refuses_what_a_decode_step_would():
+    def make(batch=2, max_len=20, **kw):
+        cfg = nsa.NSAConfig(**{**dict(d_model=64, head_dim_qk=32, head_dim_v=32, n_heads=16, n_kv_groups=16, l=2, d=2, l_prime=16), **kw})
+        return nsa.NSAPagedKVCache(cfg, batch, max_len, "cpu", torch.float32, 16, 1)
+
+    assert make(batch=4095).batch == 4095
+    with pytest.raises(ValueError, match="65535 pairs"):
+        make(batch=4096)
+    d = 1 << 20
+    assert make(batch=1, n_heads=2, n_kv_groups=1, head_dim_qk=4, head_dim_v=4, l=16, d=16, l_prime=d).config.l_prime == d
+    with pytest.raises(ValueError, match="l_prime"):
+        make(batch=1, n_heads=2, n_kv_groups=1, l_prime=d + 16)
+    with pytest.raises(ValueError, match="max_len"):
+        make(batch=1, n_heads=2, n_kv_groups=1, l=1 << 19, d=1 << 19, l_prime=1 << 19, max_len=(1 << 30) + 1)
