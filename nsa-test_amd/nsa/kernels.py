@@ -1139,6 +1139,9 @@ class NSAAttention(torch.nn.Module):
             if out is not None:
                 return self.dropout(out), None
         q, gate_logits, kv = self._paged_inputs(x)
+        width = c.head_dim_qk * _ops.compute_dtype(q.dtype).itemsize
+        if width % 16:  # (before the token joins the cache)
+            raise ValueError(f"the scoring reads rows in 16 bytes: {c.head_dim_qk} features are {width} bytes")
         cache.append(kv, new, self._compress_tokens, self._compress_weights)
         seen = cache._tokens.lengths  # a sequence without a token sees nothing
         if min(new) == 0:

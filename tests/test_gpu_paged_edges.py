@@ -38,3 +38,25 @@ def test_a_released_sequence_leaves_nothing_to_the_next(dev, dtype, kw):
         assert oa.isfinite().all() and torch.equal(oa, ob), i
         if att:
             assert all(torch.equal(ia[k], ib[k]) for k in ib), i
+
+
+@torch.no_grad()
+def test_widths_that_the_scoring_refuses_leave_the_cache(dev):
+    """A decode step whose queries the scoring does not take (rows of no 16 bytes) is refused before its
+    token joins the cache."""
+    cfg = _cfg(head_dim_qk=36, head_dim_v=32)
+    m = NSAAttention(cfg).to(dev, torch.bfloat16).eval()
+    cache = NSAPagedKVCache(cfg, 2, 100, dev, torch.bfloat16)
+    x = torch.randn(2, 40, cfg.d_model, device=dev, dtype=torch.bfloat16)
+    m.prefill(x, cache, lengths=[40, 3])
+    before = [t.clone() for t in (cache._tokens.lengths, cache._tokens.tables, cache._tail, cache.sel.k)]
+    for att in (False, True):
+        with pytest.raises(ValueError, match="16 bytes"):
+            m.decode(x[:, :1], cache, output_attentions=att)
+    assert cache.lengths == [40, 3]
+    assert all(torch.equal(s, t) for s, t in zip(before, (cache._tokens.lengths, cache._tokens.tables, cache._tail, cache.sel.k)))
+    # the same widths in fp32 are 16-byte rows
+    m = m.float()
+    cache = NSAPagedKVCache(cfg, 2, 100, dev, torch.float32)
+    m.prefill(x.float(), cache, lengths=[40, 3])
+    assert m.decode(x[:, :1].float(), cache)[0].isfinite().all() and cache.lengths == [41, 4]
