@@ -559,7 +559,7 @@ class NSAPagedKVCache:
              self.block_ends.data_ptr(), out.data_ptr(), x.stride(0), n_out, *[D] * 8, layers[8].in_features, H * dv,
              tk.tables.stride(0), bk.tables.stride(0), *kc.stride()[:3], B, H, G, D, dk, dv, layers[8].in_features,
              tk.tables.shape[1], bk.tables.shape[1], tk.n_pages, ends, max(host) or 1, c.l, c.d, c.l_prime, c.n,
-             int(bool(c.include_fixed_in_selection)), int(c.n_fixed), c.w, GATE_ACT[c.gate_mode],
+             int(bool(c.include_fixed_in_selection)), int(c.n_fixed), min(c.w, _INT_MAX), GATE_ACT[c.gate_mode],
              _lib.NSA_F32 if x.dtype is torch.float32 else _lib.NSA_BF16, 3, scale, 0]
         blocks = None
         if any(fresh):

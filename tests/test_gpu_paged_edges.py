@@ -60,3 +60,20 @@ def test_widths_that_the_scoring_refuses_leave_the_cache(dev):
     cache = NSAPagedKVCache(cfg, 2, 100, dev, torch.float32)
     m.prefill(x.float(), cache, lengths=[40, 3])
     assert m.decode(x[:, :1].float(), cache)[0].isfinite().all() and cache.lengths == [41, 4]
+
+
+@torch.no_grad()
+def test_window_of_any_size(dev):
+    """A window past 32 bits is the whole context, in the step's one call as in calls of their own."""
+    torch.manual_seed(0)
+    m = NSAAttention(_cfg(w=1 << 40)).to(dev).eval()
+    same = NSAAttention(_cfg(w=1000)).to(dev).eval()
+    same.load_state_dict(m.state_dict())
+    x = torch.randn(2, 61, 128, device=dev)
+    outs = []
+    for layer in (m, same):
+        for att in (False, True):
+            cache = NSAPagedKVCache(layer.config, 2, 100, dev, torch.float32)
+            layer.prefill(x[:, :60], cache, lengths=[60, 9])
+            outs.append(layer.decode(x[:, 60:], cache, output_attentions=att)[0])
+    assert all(torch.equal(o, outs[0]) for o in outs)
