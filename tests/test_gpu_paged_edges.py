@@ -1,8 +1,10 @@
 """GPU tests of calls at the edge of the paged 4-bit cache."""
+import math
+
 import pytest
 import torch
 
-from nsa import NSAAttention, NSAConfig, NSAPagedKVCache
+from nsa import NSAAttention, NSAConfig, NSAPagedKVCache, PagedKV4, attend_kv4, store_kv4
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +79,26 @@ def test_window_of_any_size(dev):
             layer.prefill(x[:, :60], cache, lengths=[60, 9])
             outs.append(layer.decode(x[:, 60:], cache, output_attentions=att)[0])
     assert all(torch.equal(o, outs[0]) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_off_their_alignment(dev, dtype):
+    """Queries, keys and values that start in the middle of 16 bytes: the results of aligned ones."""
+    G, H, d, N = 2, 4, 64, 24
+
+    def pair(*shape):  # the same numbers, aligned and one element into a buffer
+        n = math.prod(shape)
+        buf = torch.randn(n + 1, device=dev).to(dtype)
+        off = buf[1:].view(shape)
+        assert off.is_contiguous() and off.data_ptr() % 16
+        return off.clone(), off
+
+    k, v, q = pair(N, G, d), pair(N, G, d), pair(1, H, 1, d)
+    slots, tab = torch.arange(N, device=dev), torch.tensor([[0, 1]], device=dev, dtype=torch.int32)
+    lens = torch.tensor([N], device=dev, dtype=torch.int32)
+    pools = [PagedKV4.empty(2, 16, G, d, d, dev) for _ in range(2)]
+    for i, kv in enumerate(pools):
+        store_kv4(kv, k[i], v[i], slots)
+    assert all(torch.equal(s, t) for s, t in zip(pools[0]._tensors, pools[1]._tensors))
+    a, b = (attend_kv4(q[i], pools[0], tab, lens, 0.125) for i in range(2))
+    assert a.any() and torch.equal(a, b)
