@@ -54,8 +54,14 @@ def _rows_ok(t: torch.Tensor) -> bool:
     return all((s * es) % 16 == 0 for s in t.stride()[:-1])
 
 
+def _compact(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and 16-byte aligned (contiguous() gives back a tensor that merely starts off the alignment)."""
+    c = t.contiguous()
+    return c if not c.data_ptr() % 16 else c.clone()
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    return t if _rows_ok(t) else t.contiguous()
+    return t if _rows_ok(t) else _compact(t)
 
 
 def _pad_last(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -217,7 +223,7 @@ def attn_bwd(branch: int, q, k, v, o, do, L, M, scale: float, *, window: int = 0
     ok = _pad_last(_as(o, cdt), DV)
     dok = _pad_last(_as(do, cdt), DV)
     if ok.stride() != dok.stride() or not (_rows_ok(ok) and _rows_ok(dok)):
-        ok, dok = ok.contiguous(), dok.contiguous()
+        ok, dok = _compact(ok), _compact(dok)
     Lf = _as(L, torch.float32)
     Mf = _as(M, torch.float32)
     direct_dq = dq is not None and dq.dtype == cdt and dkw == DK and _rows_ok(dq)

@@ -93,10 +93,7 @@ def _rows16(t: torch.Tensor, cdt: torch.dtype, width: int) -> torch.Tensor:
     m = t.data_ptr()
     for x in st[:-1]:
         m |= x * (4 if cdt is torch.float32 else 2)
-    if not m & 15 and st[-1] == 1:
-        return t
-    c = t.contiguous()  # (t itself where it is one that starts off the alignment)
-    return c if not c.data_ptr() & 15 else c.clone()
+    return t if not m & 15 and st[-1] == 1 else _ops._compact(t)
 
 
 class BlockTables(NamedTuple):

@@ -8,7 +8,8 @@ import oracle
 import pytest
 import torch
 
-from nsa import NSAAttention, NSAConfig, NSAKVCache, _ops
+from nsa import (CompressionAttention, NSAAttention, NSAConfig, NSAKVCache, SelectionAttention, SlidingWindowAttention,
+                 _ops)
 from nsa.kernels import _CompressTokens, score_and_select
 from test_gpu_branches import _check, _make
 
@@ -560,3 +561,38 @@ def test_decode_step_matches_its_parts(dev, dtype, B, T0, n, gate, fixed, bias):
             assert torch.equal(a, b), i
         else:
             assert ((a.double() - b.double()).norm() / b.double().norm()).item() < (2 ** -8 if dtype == torch.bfloat16 else 1e-6)
+
+
+@pytest.mark.parametrize("branch", ["sliding", "compression", "selection"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tensors_off_their_alignment(dev, dtype, branch):
+    """Queries and the output's gradient one element into a buffer (contiguous, in the middle of 16 bytes): the
+    results of aligned ones."""
+    H, G, T, d = 4, 2, 70, 64
+    cfg = NSAConfig(d_model=64, head_dim_qk=d, head_dim_v=d, n_heads=H, n_kv_groups=G, n=4)
+    g = torch.Generator(device=dev).manual_seed(0)
+    n = T if branch != "compression" else 8
+    shapes = [(1, H, T, d), (1, G, d, n), (1, G, n, d), (1, H, T, d)]
+    ends = torch.arange(n, device=dev, dtype=torch.int32) * 8 + 3
+    idx = torch.randint(-1, 2, (1, G, T, 4), device=dev, generator=g)
+
+    def run(q, k, v, do):
+        ins = [t.detach().requires_grad_() for t in (q, k, v)]
+        if branch == "sliding":
+            o = SlidingWindowAttention.apply(*ins, 0.125, 20, cfg)
+        elif branch == "compression":
+            o = CompressionAttention.apply(*ins, ends, 0.125, cfg)
+        else:
+            o = SelectionAttention.apply(*ins, idx, 0.125, cfg)
+        return [o.detach(), *torch.autograd.grad(o, ins, do)]
+
+    def off(t):
+        y = torch.empty(t.numel() + 1, device=dev, dtype=t.dtype)[1:].view(t.shape).copy_(t)
+        assert y.is_contiguous() and y.data_ptr() % 16
+        return y
+
+    ts = [torch.randn(s, device=dev, generator=g).to(dtype) for s in shapes]
+    want = run(*ts)
+    for i in (0, 3):
+        for a, b in zip(run(*(off(t) if j == i else t for j, t in enumerate(ts))), want):
+            assert torch.equal(a, b), i

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from nsa import NSAAttention, NSAConfig, NSAPagedKVCache, PagedKV4, attend_kv4, store_kv4
+from nsa import NSAAttention, NSAConfig, NSAKVCache, NSAPagedKVCache, PagedKV4, attend_kv4, store_kv4
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,24 @@ def test_rows_off_their_alignment(dev, dtype):
     assert all(torch.equal(s, t) for s, t in zip(pools[0]._tensors, pools[1]._tensors))
     a, b = (attend_kv4(q[i], pools[0], tab, lens, 0.125) for i in range(2))
     assert a.any() and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@torch.no_grad()
+def test_tokens_off_their_alignment(dev, dtype):
+    """A token's rows that start in the middle of 16 bytes: the step of aligned ones, in either cache."""
+    cfg = _cfg()
+    torch.manual_seed(0)
+    m = NSAAttention(cfg).to(dev, dtype).eval()
+    x = torch.randn(2, 45, cfg.d_model, device=dev, dtype=dtype)
+    buf = torch.empty(2 * cfg.d_model + 1, device=dev, dtype=dtype)
+    t = buf[1:].view(2, 1, -1).copy_(x[:, :1])
+    assert t.is_contiguous() and t.data_ptr() % 16
+    for make in (NSAKVCache, NSAPagedKVCache):
+        for att in (False, True):
+            caches = [make(cfg, 2, 100, dev, dtype) for _ in range(2)]
+            outs = []
+            for c, token in zip(caches, (x[:, :1].contiguous(), t)):
+                m.prefill(x, c)
+                outs.append(m.decode(token, c, output_attentions=att)[0])
+            assert outs[0].any() and torch.equal(*outs)
