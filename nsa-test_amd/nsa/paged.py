@@ -469,6 +469,10 @@ class NSAPagedKVCache:
         """Compressed keys [B,G,dk,blocks] in the layer's dtype (zeros past a sequence's own)."""
         return self._K_cmp[:, :, :-1].transpose(-1, -2)
 
+    def _not_captured(self) -> None:
+        if self.sel._dev >= 0 and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step of an NSAPagedKVCache cannot be captured into a graph: the host keeps its lengths too")
+
     def check(self, new: Sequence[int], x: Optional[torch.Tensor] = None, config=None) -> None:
         """Raises ValueError unless sequence b has room for new[b] tokens more (and rows x are on the cache's device, a
         layer's config is the cache's), RuntimeError in a graph's capture: the host keeps the lengths too, and
@@ -479,8 +483,7 @@ class NSAPagedKVCache:
             for f in _CONFIG:
                 _need(getattr(config, f) == getattr(self.config, f),
                       f"a layer with {f} {getattr(config, f)} and a cache made for {getattr(self.config, f)}")
-        if self.sel._dev >= 0 and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("a step of an NSAPagedKVCache cannot be captured into a graph: the host keeps its lengths too")
+        self._not_captured()
         _need(len(new) == self.batch, f"{len(new)} counts for {self.batch} sequences")
         most, page, need = self.max_len, self.page_size, 0
         for b, (m, n) in enumerate(zip(self._tokens.host, new)):
@@ -623,8 +626,9 @@ class NSAPagedKVCache:
         self._K_cmp[rows, :, pos] = kc
 
     def release(self, b: int) -> None:
-        """Empties sequence b: its pages are free again."""
+        """Empties sequence b: its pages are free again (not in a graph's capture, as for a step)."""
         _need(0 <= b < self.batch, f"sequence {b} of {self.batch}")
+        self._not_captured()
         self._tokens.release(b)
         self._blocks.release(b)
         # a request without a completed block is scored against block 0, which must not be the last one's

@@ -123,3 +123,21 @@ def test_tokens_off_their_alignment(dev, dtype):
                 m.prefill(x, c)
                 outs.append(m.decode(token, c, output_attentions=att)[0])
             assert outs[0].any() and torch.equal(*outs)
+
+
+@torch.no_grad()
+def test_release_in_a_capture_is_refused(dev):
+    cfg = _cfg()
+    m = NSAAttention(cfg).to(dev).eval()
+    cache = NSAPagedKVCache(cfg, 2, 100, dev, torch.float32)
+    x = torch.randn(2, 40, cfg.d_model, device=dev)
+    m.prefill(x, cache)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            x.neg()
+            cache.release(1)
+    torch.cuda.synchronize()
+    assert cache.lengths == [40, 40] and cache._tokens.lengths.tolist() == [40, 40]
+    cache.release(1)
+    assert cache.lengths == [40, 0] and cache._tokens.lengths.tolist() == [40, 0]
