@@ -587,8 +587,8 @@ typedef struct nsa_kv4_pages {
 } nsa_kv4_pages;
 
 /* Row n of k [rows,G,dk] and v [rows,G,dv] (dtype; strides (row, group), unit feature stride,
- * 16-byte aligned rows) into slots[n]; slots below 0 or outside the pool are skipped, rows that
- * name one slot twice leave one of them there block by block.  A block's scale is 2^(floor(log2
+ * 16-byte aligned rows) into slots[n]; slots below 0 or outside the pool are skipped, the others
+ * have to differ (of one named twice, codes and scales may be of different rows).  A block's scale is 2^(floor(log2
  * amax) - 2), its elements rounded to nearest even and saturated at 6; a block with an infinity
  * or NaN becomes NaN. */
 int nsa_kv4_store(const nsa_kv4_pages* pages, const void* k, int64_t stride_kn, int64_t stride_kg, const void* v,

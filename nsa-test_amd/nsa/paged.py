@@ -194,8 +194,8 @@ def store_kv4(kv: PagedKV4, k: torch.Tensor, v: torch.Tensor, slots: torch.Tenso
     """Rows k [N,G,dk] and v [N,G,dv] into slots [N] (int64: page * page_size + offset) of the pool
     (nsa_kv4_store).  Each block of 32 features gets the scale 2^(floor(log2 max|x|) - 2) and its elements
     the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times it (ties to even, saturating); a block with an
-    infinity or NaN becomes NaN.  Slots below 0 or outside the pool are skipped; of rows that name
-    one slot twice, one of them is there, block by block."""
+    infinity or NaN becomes NaN.  Slots below 0 or outside the pool are skipped; the others of a call
+    have to differ (of a slot named twice, codes and scales may be of different rows)."""
     N, dev = slots.shape[0] if slots.dim() else 0, kv._dev
     if (k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         _refuse_grad("store_kv4")
