@@ -6,9 +6,10 @@
 // running maximum and sum.  Rows of moderate length are one workgroup's whole work (kv4_split: when).
 // Otherwise the keys of each source are cut into parts, a workgroup a part, which writes one partial
 // {max, sum, O} to the workspace; a second kernel joins the parts of each head.  The number of
-// parts is the host's (lengths are on the device, so it goes by what they may be); how many keys a
-// part holds follows on the device from the request's own count, so that a short request uses few
-// parts and a long one evenly long ones.
+// parts is the host's (lengths are on the device, so it goes by what they may be), the same for every
+// request; how many keys a part holds follows on the device from the request's own count, so that a short
+// request uses few parts.  A request much longer than the rest of its batch has no more of them
+// than they may have (kv4_split: what that costs).
 //
 // Bound, 131072 keys of H64 G4 dk 192 dv 128 (91 MB): memory while it runs, 98 MB of L2 misses in the 16 us
 // that its waves live (6.1 TB/s; the vector units are busy 42 % of that time, a wave waits for 50 %), within
@@ -20,7 +21,11 @@
 // features as long as Q's agree), turned into bf16 in registers.  V rows go through LDS as bf16 and
 // come back transposed.  Queries and probabilities in fp32 are split into three bf16 parts that hold
 // all 24 bits (x = hi + mid + lo, each the rounding of what is left): the cached values are exact in
-// bf16, so three bf16 products replace each fp32 one, at the accuracy of fp32.
+// bf16, so three bf16 products replace each fp32 one, at the accuracy of fp32.  With bf16 queries each
+// probability is rounded to bf16 for the second product (by 2^-8 of it at most; their sum is of the unrounded
+// ones, in fp32), as in the other attention kernels here: one product instead of two.  Over values of any
+// sign that adds about what rounding the output does: 2.0e-3 to 2.3e-3 from the 64-bit result (norm of the
+// difference over its norm), where that result rounded to bf16 is 1.65e-3 from it.
 #include <float.h>
 #include <limits.h>
 #include <stdio.h>
@@ -158,7 +163,8 @@ __device__ __forceinline__ float kv4_gate(int act, int s, float z0, float z1, fl
 }
 
 // waves a SIMD that a kernel's registers leave room for, and waves of a workgroup that takes a row's
-// whole work: as many as its registers and LDS allow on a CU
+// whole work: as many as its registers and LDS allow on a CU.  Held to that, some put bytes of a lane into
+// scratch: bf16 dk 192 12 (two registers; whole) and 48, fp32 dk 192 48 (whole) and 64, fp32 dk 128 48 (parts)
 __host__ __device__ constexpr int kv4_waves(int esz, int dk) { return esz == 2 ? 4 : dk == 192 ? 2 : dk == 128 ? 3 : 4; }
 __host__ __device__ constexpr int kv4_whole_waves(int esz, int dk) { return esz == 2 || dk <= 64 ? 16 : 8; }
 
@@ -669,19 +675,16 @@ static void kv4_split(const nsa_kv4_attn_args& x, Kv4Attn& a) {
     a.src[s].parts = IntDiv::make(a.parts[s]);
     a.nparts += a.parts[s];
   }
-  // A workgroup for a row's whole work, or parts and their join?  Whole: no partials and one launch, but
-  // only as many CUs at work as there are columns, 512 keys (fp32 from dk 128 on 256) a round.  Call,
-  // whole / parts in us, bf16 dk 192: 1 column 256 keys 8.2 / 8.3, 1024 11.2 / 8.9; 64 columns 1024 11.7 /
-  // 12.6, 2048 15.9 / 14.2; 128 columns 2048 16.6 / 17.6, 4096 24.2 / 22.8; 256 columns 2048 20.1 / 23.4,
-  // 4096 31.7 / 33.9; bf16 dk 64: 64 columns 1024 8.6 / 9.2, 2048 10.9 / 9.9; 256 columns 4096 16.9 / 21.5;
-  // fp32 dk 128: 64 columns 1024 12.0 / 13.1, 2048 18.2 / 15.2; 256 columns 2048 20.6 / 25.1.  So whole up to
-  // some 22 keys for each column.  A column a CU or more: at any length (lengths from a 16th to all of it,
-  // bf16 dk 192: 256 columns 8192 43 / 49, 16384 77 / 86; 512 75 / 86, 141 / 163; 1024 of 8192 134 / 153; bf16 dk 64
-  // 26 / 32, 43 / 52; 47 / 54, 80 / 99; 81 / 82; fp32 dk 128 56 / 60, 103 / 105; 100 / 107, 203 / 205; 188 / 173).  Of few
-  // columns up to 1024 keys (bf16 to dk 64 2048), though a graph's replay takes longer so: the launch less is 4 us less of the
-  // host, and a call alone takes as long either way (1024 keys, 4 columns, whole / parts: calls in a row
-  // 10.7 / 14.9, one alone 27.6 / 27.8, replayed 11.4 / 9.1; fp32 dk 128 11.2 / 13.0, 27.6 / 27.7, 11.7 / 9.2; bf16
-  // 1536 keys 12.7 / 14.6, 29.7 / 28.0, 13.3 / 9.4, bf16 dk 64 2048 10.0 / 13.0, 26.0 / 26.6, 10.5 / 8.5).
+  // A workgroup for a row's whole work, or parts and their join?  Whole is one launch, 4 us less of the host,
+  // and no partials, but a row's keys then go 512 a round (fp32 from dk 128 on 256) however many CUs are
+  // idle.  Call, whole / parts in us, bf16 dk 192: 64 columns of 1024 keys 11.7 / 12.6, of 2048 15.9 / 14.2;
+  // 128 columns of 2048 16.6 / 17.6, of 4096 24.2 / 22.8; 256 columns of 4096 31.7 / 33.9.  So whole up to some
+  // 22 keys for each column, and with a column a CU or more at any length, where lengths are within a 16th of
+  // the longest (256 columns of up to 16384 77 / 86, 512 141 / 163; fp32 dk 128 103 / 105, 203 / 205).  Of few
+  // columns up to 1024 keys (bf16 to dk 64 2048) for the host's sake (1024 keys, 4 columns: calls in a row
+  // 10.7 / 14.9, one alone 27.6 / 27.8, replayed 11.4 / 9.1).
+  // The rule sees the columns and the longest length alone, so that one long request among many short ones
+  // gets few workgroups: 131072 keys (H64 G4 bf16 dk 192) alone 26 us, among 16 requests 129, 32 248, 64 482.
   const int64_t few = x.dtype == NSA_BF16 && x.head_dim_qk <= 64 ? 2048 : 1024;
   a.whole = columns >= 256 || all <= std::max<int64_t>(few, 22 * columns);
 }
