@@ -11,8 +11,8 @@ namespace nsa {
 
 // The blocks that a step completes, one request or another nearly every step of a ragged batch: eight
 // launches over the closing requests alone, bound by their latency.  16 sequences of 8000 tokens (H32
-// G2 dk 128), a block a step: the step 117 us (74 without one), 391 with the layers over all
-// sequences by torch calls between the phases; 32 of 4000 at H64 G4 dk 192: 146 (114), 424.
+// G2 dk 128), a block a step: the step 103 us (72 without one), 391 with the layers over all
+// sequences by torch calls between the phases; 32 of 4000 at H64 G4 dk 192: 147 (113), 424.
 //
 // A token of a closing request a workgroup (i l + u: token u of the i-th such request's last l): its key of
 // the ring to k [.][l][nk], in 16-byte pieces; and fresh[z] = whether z closes a block.
